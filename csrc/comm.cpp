@@ -531,6 +531,8 @@ void register_decode(py::module_& m);
 void register_skinny(py::module_& m);
 void register_fp8(py::module_& m);
 void register_microbench(py::module_& m);
+void register_kv_cache(py::module_& m);
+void register_page_plan(py::module_& m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   using namespace sn;
@@ -619,4 +621,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_skinny(m);
   register_fp8(m);
   register_microbench(m);
+  register_kv_cache(m);
+  register_page_plan(m);
 }
