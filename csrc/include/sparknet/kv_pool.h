@@ -45,10 +45,15 @@ class KvPool {
                                                               const c10::optional<at::Tensor>& out, bool want_lse);
 
   at::Tensor k, v, k_scale, v_scale;
+  at::Tensor err;  // one int32: nonzero after a wait of the attention kernel ran out
   int64_t pages;
   int heads, page_size, dim;
 
  private:
+  CUtensorMap make_map(const at::Tensor& codes) const;
+  CUtensorMap k_map_, v_map_;  // made by the first attention call
+  bool mapped_ = false;
+
   void need_device(const at::Tensor& t, const char* what) const {
     if (t.device() != k.device()) throw std::invalid_argument(std::string(what) + " must be on the cache's device");
   }

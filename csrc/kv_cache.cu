@@ -327,6 +327,7 @@ KvPool::KvPool(at::Tensor k_, at::Tensor v_, at::Tensor ks_, at::Tensor vs_)
   need_device(k_scale, "k_scale");
   need_device(v_scale, "v_scale");
   need(aligned16(k.data_ptr()) && aligned16(v.data_ptr()), "k and v must be 16-byte aligned");
+  err = at::zeros({1}, k_scale.options().dtype(at::kInt));
 }
 
 static void need_rows(const at::Tensor& t, const char* what) {
@@ -490,6 +491,7 @@ void register_kv_cache(py::module_& m) {
       .def_readonly("v", &KvPool::v)
       .def_readonly("k_scale", &KvPool::k_scale)
       .def_readonly("v_scale", &KvPool::v_scale)
+      .def_readonly("err", &KvPool::err)
       .def_readonly("num_pages", &KvPool::pages)
       .def_readonly("kv_heads", &KvPool::heads)
       .def_readonly("page_size", &KvPool::page_size)

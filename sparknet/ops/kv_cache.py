@@ -65,6 +65,15 @@ class Fp8KVCache:
         """Bytes of the codes and scales."""
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale))
 
+    def check(self) -> None:
+        """Synchronise and raise if an attention kernel over this cache gave up on a load."""
+        if self.device.type == "cuda":
+            torch.cuda.synchronize(self.device)
+        code = int(self._pool.err.item())
+        if code:
+            self._pool.err.zero_()
+            raise RuntimeError(f"paged_decode_attention failed: error {code} (an mbarrier wait timed out)")
+
 
 def _check_slots(cache: Fp8KVCache, slots: torch.Tensor) -> None:
     """Raise if two separate runs of ``slots`` fall into one page."""

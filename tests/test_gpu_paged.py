@@ -622,12 +622,12 @@ def test_step_of_the_whole_path_and_its_graphs(device):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=side):
             outs, _ = step(table, caches, x)
-        graphs.append((graph, x, outs, table))
+        graphs.append((graph, x, outs, table, caches))  # a graph's tensors are kept as long as it
     for i, s in enumerate(steps):
-        for graph, x, outs, _ in graphs:
+        for graph, x, *_ in graphs:
             x.copy_(s)
             graph.replay()
-        for _, _, outs, _ in graphs:
+        for _, _, outs, *_ in graphs:
             assert all(torch.equal(a, b) for a, b in zip(outs, eager[i]))
     assert graphs[0][3].lengths.tolist() == [p + 6 for p in prompt]
 
