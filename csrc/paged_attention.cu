@@ -39,9 +39,8 @@ namespace {
 
 using sn::tc::smem_u32;
 
-constexpr int kWarps = 4;
 constexpr int kTile = 32;  // keys
-constexpr int kMinChunk = kWarps;  // tiles: one for each warp
+constexpr int kDirectTiles = 32;
 
 struct AttnArgs {
   const void* q;
@@ -54,7 +53,7 @@ struct AttnArgs {
   int* plan;       // [0] tiles in a chunk, [1 + b] first tile of sequence b (one KV head and row group)
   uint32_t* err;
   int64_t q_b, q_t, q_h, table_row;
-  int pages, n, T, hq, hkv, group, row_groups, page_size, width, window;
+  int pages, n, T, hq, hkv, group, row_groups, page_size, page_shift, width, window, direct;
   float scale_log2;
 };
 
@@ -64,7 +63,7 @@ struct Span {  // tiles of one sequence that some row sees
 
 __device__ __forceinline__ Span span_of(const AttnArgs& a, int b) {
   Span s;
-  s.len = min(max(a.lengths[b], 0), a.width * a.page_size);
+  s.len = min(max(a.lengths[b], 0), a.width << a.page_shift);
   s.first = a.window ? max(s.len - a.T + 1 - a.window, 0) / kTile : 0;
   s.tiles = s.len ? (s.len + kTile - 1) / kTile - s.first : 0;
   return s;
@@ -129,14 +128,18 @@ __device__ __forceinline__ void copy4(void* dst, const float* src, bool on) {
 
 template <int D, int NT>
 struct Layout {
-  static constexpr int kStages = D == 64 ? (NT == 4 ? 4 : 6) : NT == 1 ? 3 : 2;
+  // warps of a block (two blocks to an SM) and tiles in each warp's ring: as many as registers
+  // and shared memory hold
+  static constexpr int kWarps = D == 64 ? (NT == 1 ? 8 : NT == 2 ? 6 : 4) : NT == 1 ? 6 : 4;
+  static constexpr int kStages = D == 64 ? (NT == 1 ? 3 : 4) : 2;
+  static constexpr int kThreads = 32 * kWarps;
   static constexpr int kTileBytes = kTile * D;          // K or V
   static constexpr int kRing = kWarps * kStages * 2 * kTileBytes;
   static constexpr int kRows = 8 * NT;
   static constexpr int kPitch = D + 4;                  // floats; spreads the four lanes of a row over the banks
   static constexpr int kSumBytes = 2 * kRows * kPitch * 4;
   static constexpr int kQBytes = kRows * D * 2;
-  struct Stage {
+  struct alignas(16) Stage {
     float k_scale[2], v_scale[2];  // of the tile's two halves of 16 keys
     int on[2], pad[2];             // whether the half's page exists
   };
@@ -147,7 +150,7 @@ struct Layout {
 
 // A warp's place in the line of tiles.
 struct Cursor {
-  int b, hr, i, g;  // sequence; KV head * row_groups + row group; tile of the sequence; tile of the line
+  int b, h, rg, i, g;  // sequence, KV head, row group; tile of the sequence; tile of the line
   Span s;
   __device__ __forceinline__ void step(const AttnArgs& a, int by, int end) {
     g += by;
@@ -155,10 +158,13 @@ struct Cursor {
     if (g >= end) return;
     while (i >= s.tiles) {
       i -= s.tiles;
-      if (++hr == a.hkv * a.row_groups) {
-        hr = 0;
-        do s = span_of(a, ++b);
-        while (s.tiles == 0);
+      if (++rg == a.row_groups) {
+        rg = 0;
+        if (++h == a.hkv) {
+          h = 0;
+          do s = span_of(a, ++b);
+          while (s.tiles == 0);
+        }
       }
     }
   }
@@ -178,11 +184,11 @@ __device__ __forceinline__ uint32_t pair_of(float a, float b, __nv_bfloat16) { r
 __device__ __forceinline__ uint32_t pair_of(float a, float b, __half) { return pack_half2(a, b); }
 
 template <class T, int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32) k_attention(const __grid_constant__ CUtensorMap k_map,
+__global__ void __launch_bounds__(Layout<D, NT>::kThreads, 2) k_attention(const __grid_constant__ CUtensorMap k_map,
                                                            const __grid_constant__ CUtensorMap v_map,
                                                            const AttnArgs a) {
   using L = Layout<D, NT>;
-  constexpr int S = L::kStages, C = D / 16;
+  constexpr int S = L::kStages, C = D / 16, W = L::kWarps;
   extern __shared__ uint8_t raw[];
   uint8_t* ring = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
   float* sums = reinterpret_cast<float*>(ring + L::kRing);
@@ -190,8 +196,8 @@ __global__ void __launch_bounds__(kWarps * 32) k_attention(const __grid_constant
   auto* info = reinterpret_cast<typename L::Stage*>(ring + L::kRing + L::kSumBytes + L::kQBytes);
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + L::kRing + L::kSumBytes + L::kQBytes + L::kStageBytes);
   __shared__ float q_scale[L::kRows];                 // score factor of each row
-  __shared__ float sm[kWarps][L::kRows], sl[kWarps][L::kRows], sv[kWarps];
-  __shared__ int found[3], warp_tiles[kWarps];
+  __shared__ float sm[W][L::kRows], sl[W][L::kRows];
+  __shared__ int found[3], warp_tiles[W];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g8 = lane >> 2, t4 = lane & 3;
   const int hr_count = a.hkv * a.row_groups;
 
@@ -207,55 +213,68 @@ __global__ void __launch_bounds__(kWarps * 32) k_attention(const __grid_constant
       sn::tc::prefetch_tmap(&v_map);
     }
   }
-  int total = 0, chunk = 0, start = 0;
-  for (int pass = 0; pass < 2; ++pass) {  // the total, then the sequence that holds the chunk's first tile
-    if (pass) {
-      total *= hr_count;
-      chunk = max((total + int(gridDim.x) - 1) / int(gridDim.x), kMinChunk);
-      start = min(int(blockIdx.x), (total + chunk - 1) / chunk) * chunk;  // no overflow for idle blocks
-      if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[0] = chunk;
-    }
-    int before = 0;
-    for (int b0 = 0; b0 < a.n; b0 += kWarps * 32) {
-      const int b = b0 + threadIdx.x;
-      const int mine = b < a.n ? span_of(a, b).tiles : 0;
-      int sum = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o *= 2) {
-        const int up = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += up;
-      }
-      if (lane == 31) warp_tiles[warp] = sum;
-      __syncthreads();
-      int here = before;
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) here += warp_tiles[w];
-        before += warp_tiles[w];
-      }
-      __syncthreads();
-      here += sum - mine;  // tiles of the sequences before b
-      if (pass) {
-        if (b < a.n && mine && start >= here * hr_count && start < (here + mine) * hr_count) {
-          found[0] = b;
-          found[1] = here;
-          found[2] = mine;
-        }
-        if (blockIdx.x == 0 && b < a.n) a.plan[1 + b] = here;
-      }
-    }
-    if (!pass) total = before;
-    else if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[1 + a.n] = before;
-  }
-  __syncthreads();
-  const int g0 = start, g1 = min(total, start + chunk);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (g0 >= g1) return;
-
   Cursor seg;  // the segment that the block computes
-  {
-    const int rest = g0 - found[1] * hr_count;
+  int g0 = 0, g1 = 0;
+  if (a.direct) {
+    seg.b = blockIdx.x / hr_count;
+    seg.h = blockIdx.x % hr_count / a.row_groups;
+    seg.rg = blockIdx.x % a.row_groups;
+    seg.s = span_of(a, seg.b);
+    seg.i = seg.g = 0;
+    g1 = seg.s.tiles;
+    __syncthreads();
+  } else {
+    // the total, then the sequence that holds the chunk's first tile
+    int total = 0, chunk = 0, here = 0, mine = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+      int before = 0;
+      if (pass) {
+        total *= hr_count;
+        chunk = max((total + int(gridDim.x) - 1) / int(gridDim.x), W);  // a tile for each warp at least
+        g0 = min(int(blockIdx.x), (total + chunk - 1) / chunk) * chunk;  // no overflow for idle blocks
+        g1 = min(total, g0 + chunk);
+      }
+      for (int b0 = 0; b0 < a.n; b0 += L::kThreads) {
+        const int b = b0 + threadIdx.x;
+        if (!pass || a.n > L::kThreads) {
+          mine = b < a.n ? span_of(a, b).tiles : 0;
+          int sum = mine;
+#pragma unroll
+          for (int o = 1; o < 32; o *= 2) {
+            const int up = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += up;
+          }
+          if (lane == 31) warp_tiles[warp] = sum;
+          __syncthreads();
+          here = before + sum - mine;  // tiles of the sequences before b
+          for (int w = 0; w < W; ++w) {
+            if (w < warp) here += warp_tiles[w];
+            before += warp_tiles[w];
+          }
+          if (a.n > L::kThreads) __syncthreads();
+        }
+        if (pass) {
+          if (mine && g0 >= here * hr_count && g0 < (here + mine) * hr_count) {
+            found[0] = b;
+            found[1] = here;
+            found[2] = mine;
+          }
+          if (blockIdx.x == 0 && b < a.n) a.plan[1 + b] = here;
+        }
+      }
+      if (!pass) total = before;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      a.plan[0] = chunk;
+      a.plan[1 + a.n] = total / hr_count;
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (g0 >= g1) return;
+    const int rest = g0 - found[1] * hr_count, hr = rest / found[2];
     seg.b = found[0];
-    seg.hr = rest / found[2];
+    seg.h = hr / a.row_groups;
+    seg.rg = hr % a.row_groups;
     seg.i = rest % found[2];
     seg.g = g0;
     seg.s = span_of(a, seg.b);
@@ -273,16 +292,16 @@ __global__ void __launch_bounds__(kWarps * 32) k_attention(const __grid_constant
     if (c.g < g1) {
       const int key = (c.s.first + c.i) * kTile;
       const int* table = a.tables + c.b * a.table_row;
-      p.p[0] = table[key / a.page_size];
+      p.p[0] = table[key >> a.page_shift];
       p.p[1] = !halves ? p.p[0] : key + 16 < c.s.len ? table[key / 16 + 1] : -1;
     }
     return p;
   };
   auto request = [&](const Cursor& c, const Pages& p, int stage) {
     if (lane == 0 && c.g < g1) {
-      const int key = (c.s.first + c.i) * kTile, h = c.hr / a.row_groups;
+      const int place = (c.s.first + c.i) * kTile & (a.page_size - 1);
       const bool on0 = p.p[0] >= 0 && p.p[0] < a.pages, on1 = p.p[1] >= 0 && p.p[1] < a.pages;
-      const int z0 = on0 ? p.p[0] * a.hkv + h : 0, z1 = on1 ? p.p[1] * a.hkv + h : 0;
+      const int z0 = on0 ? p.p[0] * a.hkv + c.h : 0, z1 = on1 ? p.p[1] * a.hkv + c.h : 0;
       typename L::Stage& st = info[stage];
       st.on[0] = on0;
       st.on[1] = on1;
@@ -303,8 +322,8 @@ __global__ void __launch_bounds__(kWarps * 32) k_attention(const __grid_constant
           load_keys(dst + L::kTileBytes * 3 / 2, &v_map, 0, z1, &bars[stage]);
         }
       } else if (on0) {
-        load_keys(dst, &k_map, key % a.page_size, z0, &bars[stage]);
-        load_keys(dst + L::kTileBytes, &v_map, key % a.page_size, z0, &bars[stage]);
+        load_keys(dst, &k_map, place, z0, &bars[stage]);
+        load_keys(dst + L::kTileBytes, &v_map, place, z0, &bars[stage]);
       }
     }
   };
@@ -318,7 +337,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_attention(const __grid_constant
       at[s] = ahead;
       p[s] = look_up(ahead);
       pending += ahead.g < g1;
-      ahead.step(a, kWarps, g1);
+      ahead.step(a, W, g1);
     }
     next = look_up(ahead);
 #pragma unroll
@@ -329,15 +348,18 @@ __global__ void __launch_bounds__(kWarps * 32) k_attention(const __grid_constant
   int stage = 0;
   uint32_t phase = 0;
   bool dead = false;  // a load did not arrive: compute nothing more
-  // chunk c of row r of a tile lies at (c ^ swizzle(r)) * 16
-  const int mrow = (lane & 7) + ((lane >> 3) & 1) * 8, mchunk = lane >> 4;
-  const int swz = D == 128 ? lane & 7 : (lane >> 1) & 3;
-  for (bool first_segment = true; seg.g < g1; first_segment = false) {
+  // chunk c of row r of a tile lies at (c ^ swizzle(r)) * 16; this lane reads rows and chunks of
+  // its own in each 8 x 8 matrix, chunk 0's address being the base that the others differ from
+  // by an exclusive or
+  const uint32_t lane_at = ((lane & 7) + ((lane >> 3) & 1) * 8) * D +
+                           (((lane >> 4) ^ (D == 128 ? lane & 7 : (lane >> 1) & 3)) << 4);
+  bool first_segment = true;
+  do {
     const Span span = seg.s;
-    const int b = seg.b, h = seg.hr / a.row_groups, r0 = (seg.hr % a.row_groups) * L::kRows;
+    const int b = seg.b, h = seg.h, r0 = seg.rg * L::kRows;
     const int i0 = seg.i, i1 = min(span.tiles, i0 + g1 - seg.g), rows = a.T * a.group;
     // q rows to fp16 fragments
-    for (int nt = warp; nt < NT; nt += kWarps) {
+    for (int nt = warp; nt < NT; nt += W) {
       const int r = r0 + nt * 8 + g8;
       uint2 w[C];
       float amax = 0.0f;
@@ -393,13 +415,13 @@ __global__ void __launch_bounds__(kWarps * 32) k_attention(const __grid_constant
     }
     const int least = a.window ? max(span.len - a.T + 1 - a.window, 0) : 0;  // first key that any row sees
 
-    for (int i = i0 + ((warp - (seg.g - g0)) & (kWarps - 1)); i < i1; i += kWarps) {
+    for (int i = i0 + (warp + W - (seg.g - g0) % W) % W; i < i1; i += W) {
       if (!dead) dead = !sn::tc::mbar_wait(&bars[stage], phase, a.err);
       if (dead) continue;
       const int j0 = (span.first + i) * kTile;
       {
         const typename L::Stage st = info[stage];
-        const uint32_t kt = smem_u32(ring + stage * 2 * L::kTileBytes) + mrow * D, vt = kt + L::kTileBytes;
+        const uint32_t kt = smem_u32(ring + stage * 2 * L::kTileBytes) + lane_at;
         const bool edge = j0 + kTile - 1 > span.len - a.T || (a.window && j0 <= span.len - 1 - a.window) ||
                           !(st.on[0] && st.on[1]);
         // scores of two times 16 keys
@@ -413,7 +435,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_attention(const __grid_constant
 #pragma unroll
           for (int c = 0; c < C; c += 2) {
             uint32_t x[4];
-            ldsm4(kt + mt * 16 * D + (((c + mchunk) ^ swz) << 4), x);
+            ldsm4((kt ^ (c << 4)) + mt * 16 * D, x);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
               const uint32_t a0 = half2_of_codes(x[2 * u]), a1 = half2_of_codes(x[2 * u + 1]);
@@ -426,26 +448,30 @@ __global__ void __launch_bounds__(kWarps * 32) k_attention(const __grid_constant
             }
           }
         }
-        // their largest; key of element e: j0 + 16 mt + g8 + 8 (e / 2), row 2 t4 + e % 2
+        // key of element e: j0 + 16 mt + g8 + 8 (e / 2), row 2 t4 + e % 2
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[mt][nt][e] *= st.k_scale[mt] * f[nt][e & 1];
+        if (edge) {
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int key = j0 + mt * 16 + g8 + (e >> 1) * 8, last = limit[nt][e & 1];
+                if (!(key <= last && (!a.window || key > last - a.window) && st.on[mt])) s[mt][nt][e] = -INFINITY;
+              }
+        }
         float top[NT][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          top[nt][0] = top[nt][1] = -INFINITY;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float x = s[mt][nt][e] * (st.k_scale[mt] * f[nt][e & 1]);
-              if (edge) {
-                const int key = j0 + mt * 16 + g8 + (e >> 1) * 8, last = limit[nt][e & 1];
-                const bool seen = key <= last && (!a.window || key > last - a.window) && st.on[mt];
-                x = seen ? x : -INFINITY;
-              }
-              s[mt][nt][e] = x;
-              top[nt][e & 1] = fmaxf(top[nt][e & 1], x);
-            }
-          }
-        }
+          for (int e = 0; e < 2; ++e)
+            top[nt][e] = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
 #pragma unroll
         for (int x = 4; x < 32; x *= 2)
 #pragma unroll
@@ -498,40 +524,44 @@ __global__ void __launch_bounds__(kWarps * 32) k_attention(const __grid_constant
         }
         // O^T += V^T P^T; a transposed piece holds elements (2 g8, 2 g8 + 1) of keys 2 t4, 2 t4 + 1
         bool odd = false;  // a NaN code among an edge tile's keys
+        auto second = [&](auto masked) {
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-          if (edge) {  // codes of keys that no row sees may be anything: they count as zero
+          for (int mt = 0; mt < 2; ++mt) {
+            uint32_t keep[2];
+            if constexpr (masked) {  // codes of keys that no row sees may be anything: they count as zero
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int key = j0 + mt * 16 + u * 8 + t4 * 2;
-              keep[u] = (key >= least && key < span.len && st.on[mt] ? 0xffffu : 0u) |
-                        (key + 1 >= least && key + 1 < span.len && st.on[mt] ? 0xffff0000u : 0u);
-            }
-          }
-#pragma unroll
-          for (int c = 0; c < C; c += 2) {
-            uint32_t x[4];
-            ldsm4_trans(vt + mt * 16 * D + (((c + mchunk) ^ swz) << 4), x);
-            if (edge) {
-#pragma unroll
-              for (int u = 0; u < 4; ++u) {
-                x[u] &= keep[u & 1];
-                const uint32_t nan = __vcmpeq4(x[u] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                odd = odd || nan;
-                x[u] &= ~nan;  // counted below for the rows that see it
+              for (int u = 0; u < 2; ++u) {
+                const int key = j0 + mt * 16 + u * 8 + t4 * 2;
+                keep[u] = (key >= least && key < span.len && st.on[mt] ? 0xffffu : 0u) |
+                          (key + 1 >= least && key + 1 < span.len && st.on[mt] ? 0xffff0000u : 0u);
               }
             }
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const uint32_t y = __byte_perm(x[2 * u], 0, 0x3120), z = __byte_perm(x[2 * u + 1], 0, 0x3120);
-              const uint32_t a0 = half2_of_codes(y), a1 = half2_of_codes(y >> 16);
-              const uint32_t a2 = half2_of_codes(z), a3 = half2_of_codes(z >> 16);
+            for (int c = 0; c < C; c += 2) {
+              uint32_t x[4];
+              ldsm4_trans((kt ^ (c << 4)) + L::kTileBytes + mt * 16 * D, x);
+              if constexpr (masked) {
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma(o[nt][c + u], a0, a1, a2, a3, p[mt][nt][0], p[mt][nt][1]);
+                for (int u = 0; u < 4; ++u) {
+                  x[u] &= keep[u & 1];
+                  const uint32_t nan = __vcmpeq4(x[u] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                  odd = odd || nan;
+                  x[u] &= ~nan;  // counted below for the rows that see it
+                }
+              }
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const uint32_t y = __byte_perm(x[2 * u], 0, 0x3120), z = __byte_perm(x[2 * u + 1], 0, 0x3120);
+                const uint32_t a0 = half2_of_codes(y), a1 = half2_of_codes(y >> 16);
+                const uint32_t a2 = half2_of_codes(z), a3 = half2_of_codes(z >> 16);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma(o[nt][c + u], a0, a1, a2, a3, p[mt][nt][0], p[mt][nt][1]);
+              }
             }
           }
-        }
+        };
+        if (edge) second(std::true_type());
+        else second(std::false_type());
         if (edge && __any_sync(0xffffffffu, odd)) {
           // rare: how many NaN codes each (element, row) sees, as products of ones and zeros
           for (int mt = 0; mt < 2; ++mt) {
@@ -548,7 +578,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_attention(const __grid_constant
 #pragma unroll
               for (int c = 0; c < C; c += 2) {
                 uint32_t x[4];
-                ldsm4_trans(vt + mt * 16 * D + (((c + mchunk) ^ swz) << 4), x);
+                ldsm4_trans((kt ^ (c << 4)) + L::kTileBytes + mt * 16 * D, x);
 #pragma unroll
                 for (int u = 0; u < 4; ++u)  // 1.0 in e4m3 where NaN
                   x[u] = __vcmpeq4(x[u] & 0x7f7f7f7fu, 0x7f7f7f7fu) & 0x38383838u;
@@ -570,7 +600,7 @@ __global__ void __launch_bounds__(kWarps * 32) k_attention(const __grid_constant
       __syncwarp();  // every lane has read the stage
       pending += (ahead.g < g1) - 1;
       request(ahead, next, stage);
-      ahead.step(a, kWarps, g1);
+      ahead.step(a, W, g1);
       next = look_up(ahead);
       if (++stage == S) {
         stage = 0;
@@ -595,22 +625,28 @@ __global__ void __launch_bounds__(kWarps * 32) k_attention(const __grid_constant
         }
     }
     __syncthreads();
+    auto largest = [&](int r) {
+      float x = sm[0][r];
+#pragma unroll
+      for (int w = 1; w < W; ++w) x = fmaxf(x, sm[w][r]);
+      return x;
+    };
     float* mine = sums + (warp & 1) * L::kRows * L::kPitch;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {  // warps 0 and 1 store, 2 and 3 add
-      if (warp / 2 == half) {
+    for (int pair = 0; pair < W / 2; ++pair) {  // the first two warps store, the others add
+      if (warp / 2 == pair) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int r = nt * 8 + t4 * 2 + e;
-            const float best = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
+            const float best = largest(r);
             const float weight = (m[nt][e] == best ? 1.0f : ex2(m[nt][e] - best)) * vref * (1.0f / 16384.0f);
 #pragma unroll
             for (int c = 0; c < C; ++c) {
               float2* at = reinterpret_cast<float2*>(mine + r * L::kPitch + c * 16 + g8 * 2);
               float2 x = make_float2(o[nt][c][e] * weight, o[nt][c][2 + e] * weight);
-              if (half) {
+              if (pair) {
                 const float2 y = *at;
                 x.x += y.x;
                 x.y += y.y;
@@ -623,13 +659,13 @@ __global__ void __launch_bounds__(kWarps * 32) k_attention(const __grid_constant
     }
     const bool whole = i0 == 0 && i1 == span.tiles;
     const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
-    for (int x = threadIdx.x; x < L::kRows * (D / 4); x += kWarps * 32) {
+    for (int x = threadIdx.x; x < L::kRows * (D / 4); x += L::kThreads) {
       const int r = x / (D / 4), d = x % (D / 4) * 4;
       if (r0 + r >= rows) break;
-      const float best = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
+      const float best = largest(r);
       float sum = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) sum += sl[w][r] * (sm[w][r] == best ? 1.0f : ex2(sm[w][r] - best));
+      for (int w = 0; w < W; ++w) sum += sl[w][r] * (sm[w][r] == best ? 1.0f : ex2(sm[w][r] - best));
       const float4 p = *reinterpret_cast<const float4*>(sums + r * L::kPitch + d);
       const float4 q = *reinterpret_cast<const float4*>(sums + (L::kRows + r) * L::kPitch + d);
       const float4 v = make_float4(p.x + q.x, p.y + q.y, p.z + q.z, p.w + q.w);
@@ -645,8 +681,9 @@ __global__ void __launch_bounds__(kWarps * 32) k_attention(const __grid_constant
       }
     }
     __syncthreads();  // the sums and q are free for the next segment
+    first_segment = false;
     seg.step(a, i1 - i0, g1);
-  }
+  } while (seg.g < g1);
   if (dead)  // let this warp's copies land before it exits
     for (; pending > 0; --pending) {
       sn::tc::mbar_drain(&bars[stage], phase);
@@ -738,12 +775,14 @@ void launch(const AttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int
             "paged_decode_attention");
     ready.fetch_or(bit);
   }
-  kernel<<<blocks, kWarps * 32, L::kBytes, st>>>(mk, mv, a);
+  if (a.direct) blocks = a.n * a.hkv * a.row_groups;
+  kernel<<<blocks, L::kThreads, L::kBytes, st>>>(mk, mv, a);
   need_ok(cudaGetLastError(), "paged_decode_attention launch");
+  if (a.direct) return;
 
   // pieces a segment is likely cut into, four of them a group
   const int segments = a.n * a.hkv * a.row_groups, rows = std::min(L::kRows, a.T * a.group);
-  const int pieces = std::min(blocks / segments + 2, a.width * a.page_size / kTile / kMinChunk + 2);
+  const int pieces = std::min(blocks / segments + 2, a.width * a.page_size / kTile / L::kWarps + 2);
   int groups = 1;
   while (groups < 32 && groups * 4 < pieces) groups *= 2;
   int rows_here = 1;
@@ -881,6 +920,8 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> KvPool::attention(const at::Te
   a.group = int(hq / heads);
   a.row_groups = int(row_groups);
   a.page_size = page_size;
+  a.page_shift = __builtin_ctz(page_size);
+  a.direct = tables.size(1) * page_size <= kDirectTiles * kTile;
   a.width = int(tables.size(1));
   a.window = int(window);
   a.scale_log2 = float(scale * 1.4426950408889634);
