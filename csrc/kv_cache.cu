@@ -116,6 +116,7 @@ __device__ __forceinline__ void load_chunk(const T* row, int c, const float* cos
 template <class T, int D, bool ROPE>
 __global__ void __launch_bounds__(kThreads) k_append(AppendArgs a) {
   constexpr int kChunks = D / 8, kSide = kThreads / 2, kRows = kSide / kChunks;
+  constexpr int kHeld = 4;  // passes over a run that stay in registers
   __shared__ float warp_max[kThreads / 32];
   const int r0 = blockIdx.x * a.rows_per_block, r1 = min(a.n, r0 + a.rows_per_block);
   if constexpr (ROPE) {
@@ -157,121 +158,158 @@ __global__ void __launch_bounds__(kThreads) k_append(AppendArgs a) {
     }
   };
 
-  for (int r = r0; r < r1; ++r) {
-    const int slot = a.slots[r];
-    if (slot < 0 || slot >= a.slots_in_pool) continue;
-    const int place = slot % ps;
-    if (r > 0 && place != 0 && a.slots[r - 1] == slot - 1) continue;  // inside an earlier run
-    int count = 1;  // rows of the run
-    for (;;) {
-      const int j = count + lane;
-      const bool on = place + j < ps && r + j < a.n && a.slots[r + j] == slot + j;
-      const uint32_t m = __ballot_sync(0xffffffffu, on);
-      if (m == 0xffffffffu) {
-        count += 32;
-        continue;
-      }
-      count += __ffs(~m) - 1;
-      break;
-    }
-    const int64_t block = int64_t(slot / ps) * a.hkv + h;
-    float* scale_at = (is_v ? a.vs : a.ks) + block;
-    uint8_t* codes = (is_v ? a.vc : a.kc) + block * ps * D;
-    const float old = place ? *scale_at : 0.0f;
-
-    float x[8], amax = 0.0f;
-    for (int j = first; j < count; j += kRows) {
-      values(r + j, x);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float m = fabsf(x[i]);
-        amax = fmaxf(amax, m <= 3.4028234e38f ? m : 0.0f);  // finite values only
-      }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (lane == 0) warp_max[threadIdx.x / 32] = amax;
-    __syncthreads();
-    const float* wm = warp_max + (is_v ? kSide / 32 : 0);
-#pragma unroll
-    for (int i = 0; i < kSide / 32; ++i) amax = fmaxf(amax, wm[i]);
-    __syncthreads();  // warp_max is free for the next run
-    const float fresh = scale_for(amax), scale = place ? fmaxf(old, fresh) : fresh;
-    if (tid == 0) *scale_at = scale;
-
-    if (place && scale > old) {  // the older rows in the larger scale
-      const float shrink = old / scale;
-      for (int i = tid; i < place * D / 16; i += kSide) {
-        uint4* at = reinterpret_cast<uint4*>(codes) + i;
-        uint4 w = *at;
-        uint32_t* u = reinterpret_cast<uint32_t*>(&w);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 lo = values2(u[e] & 0xffffu), hi = values2(u[e] >> 16);
-          u[e] = codes2(lo.x * shrink, lo.y * shrink) | codes2(hi.x * shrink, hi.y * shrink) << 16;
+  // which of the block's rows begin a run: every warp asks for itself
+  for (int r32 = r0; r32 < r1; r32 += 32) {
+    const int own = r32 + lane < r1 ? a.slots[r32 + lane] : -1;
+    const int prior = r32 + lane < r1 && r32 + lane > 0 ? a.slots[r32 + lane - 1] : -1;
+    uint32_t begins = __ballot_sync(0xffffffffu, own >= 0 && own < a.slots_in_pool &&
+                                                     (own % ps == 0 || r32 + lane == 0 || prior != own - 1));
+    for (; begins; begins &= begins - 1) {
+      const int r = r32 + __ffs(begins) - 1, slot = __shfl_sync(0xffffffffu, own, __ffs(begins) - 1);
+      const int place = slot % ps;
+      const int64_t block = int64_t(slot / ps) * a.hkv + h;
+      float* scale_at = (is_v ? a.vs : a.ks) + block;
+      uint8_t* codes = (is_v ? a.vc : a.kc) + block * ps * D;
+      const float old = place ? *scale_at : 0.0f;
+      int count = 1;  // rows of the run
+      for (;;) {
+        const int j = count + lane;
+        const bool on = place + j < ps && r + j < a.n && a.slots[r + j] == slot + j;
+        const uint32_t m = __ballot_sync(0xffffffffu, on);
+        if (m == 0xffffffffu) {
+          count += 32;
+          continue;
         }
-        *at = w;
+        count += __ffs(~m) - 1;
+        break;
       }
-    }
-    const float inv = 1.0f / scale;
-    for (int j = first; j < count; j += kRows) {
-      if (count > kRows || j != first) values(r + j, x);  // a single pass still holds its rows
-      uint2 w;
-      w.x = codes2(x[0] * inv, x[1] * inv) | codes2(x[2] * inv, x[3] * inv) << 16;
-      w.y = codes2(x[4] * inv, x[5] * inv) | codes2(x[6] * inv, x[7] * inv) << 16;
-      *reinterpret_cast<uint2*>(codes + (place + j) * D + c * 8) = w;
+
+      float x[kHeld][8], amax = 0.0f;
+      auto load_group = [&](int j0) {
+#pragma unroll
+        for (int p = 0; p < kHeld; ++p) {
+          const int j = j0 + p * kRows + first;
+          if (j < count) values(r + j, x[p]);
+        }
+      };
+      for (int j0 = 0; j0 < count; j0 += kHeld * kRows) {
+        load_group(j0);
+#pragma unroll
+        for (int p = 0; p < kHeld; ++p)
+          if (j0 + p * kRows + first < count)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float m = fabsf(x[p][i]);
+              amax = fmaxf(amax, m <= 3.4028234e38f ? m : 0.0f);  // finite values only
+            }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      if (lane == 0) warp_max[threadIdx.x / 32] = amax;
+      __syncthreads();
+      const float* wm = warp_max + (is_v ? kSide / 32 : 0);
+#pragma unroll
+      for (int i = 0; i < kSide / 32; ++i) amax = fmaxf(amax, wm[i]);
+      __syncthreads();  // warp_max is free for the next run
+      const float fresh = scale_for(amax), scale = place ? fmaxf(old, fresh) : fresh;
+      if (tid == 0) *scale_at = scale;
+
+      if (place && scale > old) {  // the older rows in the larger scale
+        const float shrink = old / scale;
+        for (int i = tid; i < place * D / 16; i += kSide) {
+          uint4* at = reinterpret_cast<uint4*>(codes) + i;
+          uint4 w = *at;
+          uint32_t* u = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 lo = values2(u[e] & 0xffffu), hi = values2(u[e] >> 16);
+            u[e] = codes2(lo.x * shrink, lo.y * shrink) | codes2(hi.x * shrink, hi.y * shrink) << 16;
+          }
+          *at = w;
+        }
+      }
+      const float inv = 1.0f / scale;
+      for (int j0 = 0; j0 < count; j0 += kHeld * kRows) {
+        if (count > kHeld * kRows) load_group(j0);  // a run of one group is still held
+#pragma unroll
+        for (int p = 0; p < kHeld; ++p) {
+          const int j = j0 + p * kRows + first;
+          if (j < count) {
+            uint2 w;
+            w.x = codes2(x[p][0] * inv, x[p][1] * inv) | codes2(x[p][2] * inv, x[p][3] * inv) << 16;
+            w.y = codes2(x[p][4] * inv, x[p][5] * inv) | codes2(x[p][6] * inv, x[p][7] * inv) << 16;
+            *reinterpret_cast<uint2*>(codes + (place + j) * D + c * 8) = w;
+          }
+        }
+      }
     }
   }
 }
 
 // --- read: slots -> rows of K and V -------------------------------------------------------
-template <class O>
-__device__ __forceinline__ void store8(O* p, const float (&x)[8]) {
-  uint4 w;
-  w.x = from_float2(x[0], x[1], O());
-  w.y = from_float2(x[2], x[3], O());
-  w.z = from_float2(x[4], x[5], O());
-  w.w = from_float2(x[6], x[7], O());
-  *reinterpret_cast<uint4*>(p) = w;
-}
-__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+// 8 words to a 32-byte aligned address, one sector at once.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 
-// Thread: 8 elements of K and of V of one (row, head).  Rows without a slot read as zeros.
+// 16 codes times `scale` to 16 values.
+template <class O>
+__device__ __forceinline__ void store16(O* p, uint4 codes, float scale) {
+  const uint32_t u[4] = {codes.x, codes.y, codes.z, codes.w};
+  uint32_t w[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 a = values2(u[e] & 0xffffu), b = values2(u[e] >> 16);
+    w[2 * e] = from_float2(a.x * scale, a.y * scale, O());
+    w[2 * e + 1] = from_float2(b.x * scale, b.y * scale, O());
+  }
+  store32(p, w);
+}
+template <>
+__device__ __forceinline__ void store16<float>(float* p, uint4 codes, float scale) {
+  const uint32_t u[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    uint32_t w[8];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float2 a = values2(u[2 * g + e] & 0xffffu), b = values2(u[2 * g + e] >> 16);
+      w[4 * e] = __float_as_uint(a.x * scale);
+      w[4 * e + 1] = __float_as_uint(a.y * scale);
+      w[4 * e + 2] = __float_as_uint(b.x * scale);
+      w[4 * e + 3] = __float_as_uint(b.y * scale);
+    }
+    store32(p + 8 * g, w);
+  }
+}
+
+// Thread: 16 elements of K and of V of one (row, head).  Rows without a slot read as zeros.
 template <class O, int D>
 __global__ void __launch_bounds__(kThreads) k_read(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
                                                    const float* __restrict__ ks, const float* __restrict__ vs,
                                                    const int* __restrict__ slots, O* __restrict__ k_out,
-                                                   O* __restrict__ v_out, int64_t total, int hkv, int page_size,
+                                                   O* __restrict__ v_out, int64_t total, int hkv, int page_shift,
                                                    int64_t slots_in_pool) {
-  constexpr int kChunks = D / 8;
-  for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < total; i += int64_t(gridDim.x) * kThreads) {
-    const int c = int(i % kChunks);
-    const int64_t rh = i / kChunks;
-    const int h = int(rh % hkv);
-    const int slot = slots[rh / hkv];
-    float x[8] = {}, y[8] = {};
-    if (slot >= 0 && slot < slots_in_pool) {
-      const int64_t block = int64_t(slot / page_size) * hkv + h;
-      const int64_t at = (block * page_size + slot % page_size) * D + c * 8;
-      const uint2 kw = *reinterpret_cast<const uint2*>(kc + at), vw = *reinterpret_cast<const uint2*>(vc + at);
-      const float a = ks[block], b = vs[block];
-      const uint32_t ku[4] = {kw.x & 0xffffu, kw.x >> 16, kw.y & 0xffffu, kw.y >> 16};
-      const uint32_t vu[4] = {vw.x & 0xffffu, vw.x >> 16, vw.y & 0xffffu, vw.y >> 16};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 p = values2(ku[e]), q = values2(vu[e]);
-        x[2 * e] = p.x * a;
-        x[2 * e + 1] = p.y * a;
-        y[2 * e] = q.x * b;
-        y[2 * e + 1] = q.y * b;
-      }
-    }
-    store8(k_out + i * 8, x);
-    store8(v_out + i * 8, y);
+  constexpr int kChunks = D / 16;
+  const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+  if (i >= total) return;
+  const int c = int(i % kChunks);
+  const int64_t rh = i / kChunks, row = total < (int64_t(1) << 31) ? int64_t(uint32_t(rh) / uint32_t(hkv)) : rh / hkv;
+  const int h = int(rh - row * hkv), slot = slots[row];
+  uint4 kw = make_uint4(0, 0, 0, 0), vw = kw;
+  float a = 0.0f, b = 0.0f;
+  if (slot >= 0 && slot < slots_in_pool) {
+    const int64_t block = int64_t(slot >> page_shift) * hkv + h;
+    const int64_t at = ((block << page_shift) + (slot & ((1 << page_shift) - 1))) * D + c * 16;
+    kw = *reinterpret_cast<const uint4*>(kc + at);
+    vw = *reinterpret_cast<const uint4*>(vc + at);
+    a = ks[block];
+    b = vs[block];
   }
+  store16(k_out + i * 16, kw, a);
+  store16(v_out + i * 16, vw, b);
 }
 
 template <class T, int D, bool ROPE>
@@ -441,8 +479,9 @@ std::tuple<at::Tensor, at::Tensor> KvPool::read(const at::Tensor& slots, at::Sca
   for (const auto* o : {&k_out, &v_out})
     if (*o)
       need((*o)->dim() == 3 && (*o)->size(0) == n && (*o)->size(1) == heads && (*o)->size(2) == dim &&
-               (*o)->scalar_type() == dtype && (*o)->is_contiguous() && aligned16((*o)->data_ptr()),
-           "k_out and v_out must be contiguous [n, kv_heads, head_dim] of the given dtype");
+               (*o)->scalar_type() == dtype && (*o)->is_contiguous() &&
+               (reinterpret_cast<uintptr_t>((*o)->data_ptr()) & 31) == 0,
+           "k_out and v_out must be contiguous, 32-byte aligned [n, kv_heads, head_dim] of the given dtype");
   need_device(slots, "slots");
   if (k_out) need_device(*k_out, "k_out");
   if (v_out) need_device(*v_out, "v_out");
@@ -451,15 +490,16 @@ std::tuple<at::Tensor, at::Tensor> KvPool::read(const at::Tensor& slots, at::Sca
   const auto options = k.options().dtype(dtype);
   at::Tensor ko = k_out ? *k_out : at::empty({n, heads, dim}, options);
   at::Tensor vo = v_out ? *v_out : at::empty({n, heads, dim}, options);
-  const int64_t total = n * heads * (dim / 8);
+  const int64_t total = n * heads * (dim / 16);
   if (total == 0) return {ko, vo};
-  const int grid = int(std::min<int64_t>((total + kThreads - 1) / kThreads, 148 * 16));
+  need((total + kThreads - 1) / kThreads <= INT32_MAX, "too many rows");
+  const int grid = int((total + kThreads - 1) / kThreads);
   auto go = [&](auto zero, auto d) {
     using O = decltype(zero);
     k_read<O, decltype(d)::value><<<grid, kThreads, 0, stream()>>>(
         static_cast<const uint8_t*>(k.data_ptr()), static_cast<const uint8_t*>(v.data_ptr()),
         k_scale.data_ptr<float>(), v_scale.data_ptr<float>(), slots.data_ptr<int>(), static_cast<O*>(ko.data_ptr()),
-        static_cast<O*>(vo.data_ptr()), total, heads, page_size, pages * page_size);
+        static_cast<O*>(vo.data_ptr()), total, heads, __builtin_ctz(page_size), pages * page_size);
   };
   auto by_dim = [&](auto zero) {
     if (dim == 128) go(zero, std::integral_constant<int, 128>());

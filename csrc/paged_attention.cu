@@ -40,7 +40,9 @@ namespace {
 using sn::tc::smem_u32;
 
 constexpr int kTile = 32;  // keys
-constexpr int kDirectTiles = 32;
+// What a segment's beginning and end cost, in rounds of a block's warps over tiles: with 0, 1, 2
+// and 3 rounds 64 ragged sequences to 8192 took 114, 99, 93 and 91 us.
+constexpr int kPadRounds = 3;
 
 struct AttnArgs {
   const void* q;
@@ -50,10 +52,10 @@ struct AttnArgs {
   const int *tables, *lengths;
   float* part;     // [2 * blocks][rows][D] sums of weighted values
   float2* part_ml; // [2 * blocks][rows] (max in log2, sum)
-  int* plan;       // [0] tiles in a chunk, [1 + b] first tile of sequence b (one KV head and row group)
+  int* plan;       // places in a chunk, then each sequence's first place (one KV head and row group), and the end
   uint32_t* err;
   int64_t q_b, q_t, q_h, table_row;
-  int pages, n, T, hq, hkv, group, row_groups, page_size, page_shift, width, window, direct;
+  int pages, n, T, hq, hkv, group, row_groups, page_size, page_shift, width, window, direct, pad, resident;
   float scale_log2;
 };
 
@@ -75,10 +77,14 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ uint32_t half2_of_codes(uint32_t codes) {  // the low 16 bits
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(codes)));
-  return h;
+// Four codes to two pairs of fp16.
+__device__ __forceinline__ void halves_of_codes(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\t"
+      "mov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(codes));
 }
 
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
@@ -148,16 +154,17 @@ struct Layout {
   static constexpr int kBytes = 1024 + kRing + kSumBytes + kQBytes + kStageBytes + kBarBytes;
 };
 
-// A warp's place in the line of tiles.
+// A place in the line.  A segment takes as many places as it has tiles, and `pad` more that
+// stand for the time of its beginning and end.
 struct Cursor {
-  int b, h, rg, i, g;  // sequence, KV head, row group; tile of the sequence; tile of the line
+  int b, h, rg, i, g;  // sequence, KV head, row group; place in the segment; place in the line
   Span s;
   __device__ __forceinline__ void step(const AttnArgs& a, int by, int end) {
     g += by;
     i += by;
     if (g >= end) return;
-    while (i >= s.tiles) {
-      i -= s.tiles;
+    while (i >= s.tiles + a.pad) {
+      i -= s.tiles + a.pad;
       if (++rg == a.row_groups) {
         rg = 0;
         if (++h == a.hkv) {
@@ -168,7 +175,44 @@ struct Cursor {
       }
     }
   }
+  // the next place that is a tile
+  __device__ __forceinline__ void settle(const AttnArgs& a, int by, int end) {
+    while (g < end && i >= s.tiles) step(a, by, end);
+  }
 };
+
+__device__ __forceinline__ int cluster_rank() {
+  int r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ int cluster_size() {
+  int r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();  // the aligned form wants whole warps
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of this block's `p` in the shared memory of block `rank` of the cluster.
+__device__ __forceinline__ uint32_t in_block(const void* p, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
+  return v;
+}
 
 template <class T>
 __device__ __forceinline__ float2 floats_of(uint32_t w);
@@ -197,6 +241,7 @@ __global__ void __launch_bounds__(Layout<D, NT>::kThreads, 2) k_attention(const 
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + L::kRing + L::kSumBytes + L::kQBytes + L::kStageBytes);
   __shared__ float q_scale[L::kRows];                 // score factor of each row
   __shared__ float sm[W][L::kRows], sl[W][L::kRows];
+  __shared__ float2 block_ml[L::kRows];               // (max, sum) of the block, for its cluster
   __shared__ int found[3], warp_tiles[W];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g8 = lane >> 2, t4 = lane & 3;
   const int hr_count = a.hkv * a.row_groups;
@@ -215,13 +260,22 @@ __global__ void __launch_bounds__(Layout<D, NT>::kThreads, 2) k_attention(const 
   }
   Cursor seg;  // the segment that the block computes
   int g0 = 0, g1 = 0;
+  int split = 1, part = 0;  // blocks of a cluster that share the segment, and this one's place among them
   if (a.direct) {
-    seg.b = blockIdx.x / hr_count;
-    seg.h = blockIdx.x % hr_count / a.row_groups;
-    seg.rg = blockIdx.x % a.row_groups;
+    if (a.direct > 1) {
+      split = cluster_size();
+      part = cluster_rank();
+      // launched without its cluster: the first block of each does it all
+      if (split != a.direct && blockIdx.x % a.direct) return;
+    }
+    const int segment = blockIdx.x / a.direct;
+    seg.b = segment / hr_count;
+    seg.h = segment % hr_count / a.row_groups;
+    seg.rg = segment % a.row_groups;
     seg.s = span_of(a, seg.b);
-    seg.i = seg.g = 0;
-    g1 = seg.s.tiles;
+    const int share = (seg.s.tiles + split - 1) / split;
+    g0 = seg.i = seg.g = min(part * share, seg.s.tiles);
+    g1 = min(g0 + share, seg.s.tiles);
     __syncthreads();
   } else {
     // the total, then the sequence that holds the chunk's first tile
@@ -231,13 +285,14 @@ __global__ void __launch_bounds__(Layout<D, NT>::kThreads, 2) k_attention(const 
       if (pass) {
         total *= hr_count;
         chunk = max((total + int(gridDim.x) - 1) / int(gridDim.x), W);  // a tile for each warp at least
-        g0 = min(int(blockIdx.x), (total + chunk - 1) / chunk) * chunk;  // no overflow for idle blocks
+        g0 = min(int(blockIdx.x) * chunk, total);
         g1 = min(total, g0 + chunk);
       }
       for (int b0 = 0; b0 < a.n; b0 += L::kThreads) {
         const int b = b0 + threadIdx.x;
         if (!pass || a.n > L::kThreads) {
           mine = b < a.n ? span_of(a, b).tiles : 0;
+          mine += mine ? a.pad : 0;
           int sum = mine;
 #pragma unroll
           for (int o = 1; o < 32; o *= 2) {
@@ -246,7 +301,7 @@ __global__ void __launch_bounds__(Layout<D, NT>::kThreads, 2) k_attention(const 
           }
           if (lane == 31) warp_tiles[warp] = sum;
           __syncthreads();
-          here = before + sum - mine;  // tiles of the sequences before b
+          here = before + sum - mine;  // places of the sequences before b
           for (int w = 0; w < W; ++w) {
             if (w < warp) here += warp_tiles[w];
             before += warp_tiles[w];
@@ -281,6 +336,7 @@ __global__ void __launch_bounds__(Layout<D, NT>::kThreads, 2) k_attention(const 
   }
   Cursor ahead = seg;  // the next tile that this warp requests
   ahead.step(a, warp, g1);
+  ahead.settle(a, W, g1);
 
   // --- requests ---------------------------------------------------------------------------
   const bool halves = a.page_size == 16;  // a tile is two pages
@@ -293,37 +349,44 @@ __global__ void __launch_bounds__(Layout<D, NT>::kThreads, 2) k_attention(const 
       const int key = (c.s.first + c.i) * kTile;
       const int* table = a.tables + c.b * a.table_row;
       p.p[0] = table[key >> a.page_shift];
-      p.p[1] = !halves ? p.p[0] : key + 16 < c.s.len ? table[key / 16 + 1] : -1;
+      p.p[1] = halves && key + 16 < c.s.len ? table[(key >> 4) + 1] : -1;
     }
     return p;
   };
   auto request = [&](const Cursor& c, const Pages& p, int stage) {
     if (lane == 0 && c.g < g1) {
-      const int place = (c.s.first + c.i) * kTile & (a.page_size - 1);
-      const bool on0 = p.p[0] >= 0 && p.p[0] < a.pages, on1 = p.p[1] >= 0 && p.p[1] < a.pages;
-      const int z0 = on0 ? p.p[0] * a.hkv + c.h : 0, z1 = on1 ? p.p[1] * a.hkv + c.h : 0;
       typename L::Stage& st = info[stage];
-      st.on[0] = on0;
-      st.on[1] = on1;
-      copy4(&st.k_scale[0], a.ks + z0, on0);
-      copy4(&st.k_scale[1], a.ks + z1, on1);
-      copy4(&st.v_scale[0], a.vs + z0, on0);
-      copy4(&st.v_scale[1], a.vs + z1, on1);
-      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bars[stage])) : "memory");
-      sn::tc::mbar_expect_tx(&bars[stage], (on0 ? L::kTileBytes : 0) + (on1 ? L::kTileBytes : 0));
+      uint64_t* bar = &bars[stage];
       const uint32_t dst = smem_u32(ring + stage * 2 * L::kTileBytes);
-      if (halves) {
+      const bool on0 = uint32_t(p.p[0]) < uint32_t(a.pages);
+      const int z0 = on0 ? p.p[0] * a.hkv + c.h : 0;
+      st.on[0] = on0;
+      copy4(&st.k_scale[0], a.ks + z0, on0);
+      copy4(&st.v_scale[0], a.vs + z0, on0);
+      if (!halves) {
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+        sn::tc::mbar_expect_tx(bar, on0 ? 2 * L::kTileBytes : 0);
         if (on0) {
-          load_keys(dst, &k_map, 0, z0, &bars[stage]);
-          load_keys(dst + L::kTileBytes, &v_map, 0, z0, &bars[stage]);
+          const int place = (c.s.first + c.i) * kTile & (a.page_size - 1);
+          load_keys(dst, &k_map, place, z0, bar);
+          load_keys(dst + L::kTileBytes, &v_map, place, z0, bar);
+        }
+      } else {
+        const bool on1 = uint32_t(p.p[1]) < uint32_t(a.pages);
+        const int z1 = on1 ? p.p[1] * a.hkv + c.h : 0;
+        st.on[1] = on1;
+        copy4(&st.k_scale[1], a.ks + z1, on1);
+        copy4(&st.v_scale[1], a.vs + z1, on1);
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+        sn::tc::mbar_expect_tx(bar, (on0 ? L::kTileBytes : 0) + (on1 ? L::kTileBytes : 0));
+        if (on0) {
+          load_keys(dst, &k_map, 0, z0, bar);
+          load_keys(dst + L::kTileBytes, &v_map, 0, z0, bar);
         }
         if (on1) {
-          load_keys(dst + L::kTileBytes / 2, &k_map, 0, z1, &bars[stage]);
-          load_keys(dst + L::kTileBytes * 3 / 2, &v_map, 0, z1, &bars[stage]);
+          load_keys(dst + L::kTileBytes / 2, &k_map, 0, z1, bar);
+          load_keys(dst + L::kTileBytes * 3 / 2, &v_map, 0, z1, bar);
         }
-      } else if (on0) {
-        load_keys(dst, &k_map, place, z0, &bars[stage]);
-        load_keys(dst + L::kTileBytes, &v_map, place, z0, &bars[stage]);
       }
     }
   };
@@ -338,6 +401,7 @@ __global__ void __launch_bounds__(Layout<D, NT>::kThreads, 2) k_attention(const 
       p[s] = look_up(ahead);
       pending += ahead.g < g1;
       ahead.step(a, W, g1);
+      ahead.settle(a, W, g1);
     }
     next = look_up(ahead);
 #pragma unroll
@@ -353,42 +417,54 @@ __global__ void __launch_bounds__(Layout<D, NT>::kThreads, 2) k_attention(const 
   // by an exclusive or
   const uint32_t lane_at = ((lane & 7) + ((lane >> 3) & 1) * 8) * D +
                            (((lane >> 4) ^ (D == 128 ? lane & 7 : (lane >> 1) & 3)) << 4);
-  bool first_segment = true;
+  // A segment's q rows, brought to fp16 fragments in shared memory by the first NT warps (W is
+  // at least NT): loaded before the previous segment's warps are joined, stored after.
+  const int rows = a.T * a.group;
+  uint2 q_raw[C];
+  auto load_q = [&](const Cursor& c) {
+    const int r = c.rg * L::kRows + warp * 8 + g8;
+#pragma unroll
+    for (int i = 0; i < C; ++i) q_raw[i] = make_uint2(0, 0);
+    if (warp < NT && r < rows) {
+      const int t = r / a.group;
+      const T* q = static_cast<const T*>(a.q) + c.b * a.q_b + t * a.q_t + (c.h * a.group + r - t * a.group) * a.q_h;
+#pragma unroll
+      for (int i = 0; i < C; ++i) q_raw[i] = *reinterpret_cast<const uint2*>(q + i * 16 + t4 * 4);
+    }
+  };
+  auto store_q = [&]() {
+    if (warp >= NT) return;
+    float amax = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const float2 x = floats_of<T>(q_raw[c].x), y = floats_of<T>(q_raw[c].y);
+      amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(y.x), fabsf(y.y)));
+    }
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    // the row's largest to [2^14, 2^15); an infinite row keeps its values
+    const int e = amax <= 3.4028234e38f ? max((__float_as_int(amax) >> 23) - 127, -100) : 14;
+    const float up = __int_as_float((14 - e + 127) << 23);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const float2 x = floats_of<T>(q_raw[c].x), y = floats_of<T>(q_raw[c].y);
+      qs[(warp * C + c) * 32 + lane] = make_uint2(pack_half2(x.x * up, x.y * up), pack_half2(y.x * up, y.y * up));
+    }
+    if (t4 == 0) q_scale[warp * 8 + g8] = a.scale_log2 * __int_as_float((e - 14 + 127) << 23);
+  };
+  auto skip_empty = [&](Cursor& c) {  // past a segment of whose places only the pad is here
+    while (c.g < g1 && c.i >= c.s.tiles) c.step(a, min(c.s.tiles + a.pad - c.i, g1 - c.g), g1);
+  };
+  if (!a.direct) skip_empty(seg);
+  if (!a.direct && seg.g >= g1) return;
+  load_q(seg);
+  store_q();
+  __syncthreads();
   do {
+    const int places = min(seg.s.tiles + a.pad - seg.i, g1 - seg.g);
     const Span span = seg.s;
     const int b = seg.b, h = seg.h, r0 = seg.rg * L::kRows;
-    const int i0 = seg.i, i1 = min(span.tiles, i0 + g1 - seg.g), rows = a.T * a.group;
-    // q rows to fp16 fragments
-    for (int nt = warp; nt < NT; nt += W) {
-      const int r = r0 + nt * 8 + g8;
-      uint2 w[C];
-      float amax = 0.0f;
-#pragma unroll
-      for (int c = 0; c < C; ++c) w[c] = make_uint2(0, 0);
-      if (r < rows) {
-        const T* q = static_cast<const T*>(a.q) + b * a.q_b + r / a.group * a.q_t + (h * a.group + r % a.group) * a.q_h;
-#pragma unroll
-        for (int c = 0; c < C; ++c) w[c] = *reinterpret_cast<const uint2*>(q + c * 16 + t4 * 4);
-      }
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const float2 x = floats_of<T>(w[c].x), y = floats_of<T>(w[c].y);
-        amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(y.x), fabsf(y.y)));
-      }
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      // the row's largest to [2^14, 2^15); an infinite row keeps its values
-      const int e = amax <= 3.4028234e38f ? max((__float_as_int(amax) >> 23) - 127, -100) : 14;
-      const float up = __int_as_float((14 - e + 127) << 23);
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const float2 x = floats_of<T>(w[c].x), y = floats_of<T>(w[c].y);
-        qs[(nt * C + c) * 32 + lane] = make_uint2(pack_half2(x.x * up, x.y * up), pack_half2(y.x * up, y.y * up));
-      }
-      if (t4 == 0) q_scale[nt * 8 + g8] = a.scale_log2 * __int_as_float((e - 14 + 127) << 23);
-    }
-    __syncthreads();
-
+    const int i0 = seg.i, i1 = min(span.tiles, i0 + places);
     uint2 qf[NT <= 2 ? NT : 1][C];
     if constexpr (NT <= 2) {
 #pragma unroll
@@ -420,7 +496,12 @@ __global__ void __launch_bounds__(Layout<D, NT>::kThreads, 2) k_attention(const 
       if (dead) continue;
       const int j0 = (span.first + i) * kTile;
       {
-        const typename L::Stage st = info[stage];
+        typename L::Stage st = info[stage];
+        if (!halves) {
+          st.k_scale[1] = st.k_scale[0];
+          st.v_scale[1] = st.v_scale[0];
+          st.on[1] = st.on[0];
+        }
         const uint32_t kt = smem_u32(ring + stage * 2 * L::kTileBytes) + lane_at;
         const bool edge = j0 + kTile - 1 > span.len - a.T || (a.window && j0 <= span.len - 1 - a.window) ||
                           !(st.on[0] && st.on[1]);
@@ -438,8 +519,9 @@ __global__ void __launch_bounds__(Layout<D, NT>::kThreads, 2) k_attention(const 
             ldsm4((kt ^ (c << 4)) + mt * 16 * D, x);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              const uint32_t a0 = half2_of_codes(x[2 * u]), a1 = half2_of_codes(x[2 * u + 1]);
-              const uint32_t a2 = half2_of_codes(x[2 * u] >> 16), a3 = half2_of_codes(x[2 * u + 1] >> 16);
+              uint32_t a0, a1, a2, a3;
+              halves_of_codes(x[2 * u], a0, a2);
+              halves_of_codes(x[2 * u + 1], a1, a3);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 const uint2 q = NT <= 2 ? qf[NT <= 2 ? nt : 0][c + u] : qs[(nt * C + c + u) * 32 + lane];
@@ -551,9 +633,9 @@ __global__ void __launch_bounds__(Layout<D, NT>::kThreads, 2) k_attention(const 
               }
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
-                const uint32_t y = __byte_perm(x[2 * u], 0, 0x3120), z = __byte_perm(x[2 * u + 1], 0, 0x3120);
-                const uint32_t a0 = half2_of_codes(y), a1 = half2_of_codes(y >> 16);
-                const uint32_t a2 = half2_of_codes(z), a3 = half2_of_codes(z >> 16);
+                uint32_t a0, a1, a2, a3;
+                halves_of_codes(__byte_perm(x[2 * u], 0, 0x3120), a0, a1);
+                halves_of_codes(__byte_perm(x[2 * u + 1], 0, 0x3120), a2, a3);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) mma(o[nt][c + u], a0, a1, a2, a3, p[mt][nt][0], p[mt][nt][1]);
               }
@@ -584,10 +666,11 @@ __global__ void __launch_bounds__(Layout<D, NT>::kThreads, 2) k_attention(const 
                   x[u] = __vcmpeq4(x[u] & 0x7f7f7f7fu, 0x7f7f7f7fu) & 0x38383838u;
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                  const uint32_t y = __byte_perm(x[2 * u], 0, 0x3120), z = __byte_perm(x[2 * u + 1], 0, 0x3120);
+                  uint32_t a0, a1, a2, a3;
+                  halves_of_codes(__byte_perm(x[2 * u], 0, 0x3120), a0, a1);
+                  halves_of_codes(__byte_perm(x[2 * u + 1], 0, 0x3120), a2, a3);
                   float hits[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                  mma(hits, half2_of_codes(y), half2_of_codes(y >> 16), half2_of_codes(z), half2_of_codes(z >> 16), b0,
-                      b1);
+                  mma(hits, a0, a1, a2, a3, b0, b1);
 #pragma unroll
                   for (int e = 0; e < 4; ++e)
                     if (hits[e] > 0.0f) o[nt][c + u][e] = NAN;
@@ -601,12 +684,18 @@ __global__ void __launch_bounds__(Layout<D, NT>::kThreads, 2) k_attention(const 
       pending += (ahead.g < g1) - 1;
       request(ahead, next, stage);
       ahead.step(a, W, g1);
+      ahead.settle(a, W, g1);
       next = look_up(ahead);
       if (++stage == S) {
         stage = 0;
         phase ^= 1;
       }
     }
+
+    Cursor following = seg;
+    following.step(a, places, g1);
+    if (!a.direct) skip_empty(following);
+    if (following.g < g1) load_q(following);
 
     // --- join the warps ---------------------------------------------------------------------
 #pragma unroll
@@ -657,8 +746,16 @@ __global__ void __launch_bounds__(Layout<D, NT>::kThreads, 2) k_attention(const 
       }
       __syncthreads();
     }
-    const bool whole = i0 == 0 && i1 == span.tiles;
-    const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
+    const bool whole = (i0 == 0 && i1 == span.tiles) || split > 1;
+    const int slot = 2 * blockIdx.x + (g0 >= seg.g - i0 ? 0 : 1);  // at most the first and the last are pieces
+    auto write = [&](int r, int d, const float4& v, float best, float sum) {
+      const int t = (r0 + r) / a.group;
+      const int64_t row = (int64_t(b) * a.T + t) * a.hq + h * a.group + r0 + r - t * a.group;
+      const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + row * D + d) =
+          make_uint2(pair_of(v.x * inv, v.y * inv, T()), pair_of(v.z * inv, v.w * inv, T()));
+      if (a.lse && d == 0) a.lse[row] = sum != 0.0f ? (best + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+    };
     for (int x = threadIdx.x; x < L::kRows * (D / 4); x += L::kThreads) {
       const int r = x / (D / 4), d = x % (D / 4) * 4;
       if (r0 + r >= rows) break;
@@ -669,20 +766,41 @@ __global__ void __launch_bounds__(Layout<D, NT>::kThreads, 2) k_attention(const 
       const float4 p = *reinterpret_cast<const float4*>(sums + r * L::kPitch + d);
       const float4 q = *reinterpret_cast<const float4*>(sums + (L::kRows + r) * L::kPitch + d);
       const float4 v = make_float4(p.x + q.x, p.y + q.y, p.z + q.z, p.w + q.w);
-      if (whole) {
-        const int64_t row = (int64_t(b) * a.T + (r0 + r) / a.group) * a.hq + h * a.group + (r0 + r) % a.group;
-        const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + row * D + d) =
-            make_uint2(pair_of(v.x * inv, v.y * inv, T()), pair_of(v.z * inv, v.w * inv, T()));
-        if (a.lse && d == 0) a.lse[row] = sum != 0.0f ? (best + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+      if (split > 1) {
+        *reinterpret_cast<float4*>(sums + r * L::kPitch + d) = v;
+        if (d == 0) block_ml[r] = make_float2(best, sum);
+      } else if (whole) {
+        write(r, d, v, best, sum);
       } else {
         *reinterpret_cast<float4*>(a.part + (int64_t(slot) * L::kRows + r) * D + d) = v;
         if (d == 0) a.part_ml[slot * L::kRows + r] = make_float2(best, sum);
       }
     }
-    __syncthreads();  // the sums and q are free for the next segment
-    first_segment = false;
-    seg.step(a, i1 - i0, g1);
+    if (split > 1) {  // join the blocks: each writes every split-th piece of the rows
+      cluster_sync();
+      for (int x = part * L::kThreads + threadIdx.x; x < L::kRows * (D / 4); x += split * L::kThreads) {
+        const int r = x / (D / 4), d = x % (D / 4) * 4;
+        if (r0 + r >= rows) break;
+        float best = -INFINITY, sum = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int c = 0; c < split; ++c) best = fmaxf(best, ld_cluster2(in_block(&block_ml[r], c)).x);
+        for (int c = 0; c < split; ++c) {
+          const float2 ml = ld_cluster2(in_block(&block_ml[r], c));
+          const float4 y = ld_cluster4(in_block(sums + r * L::kPitch + d, c));
+          const float w = ml.x == best ? 1.0f : ex2(ml.x - best);
+          sum += ml.y * w;
+          v.x += y.x * w;
+          v.y += y.y * w;
+          v.z += y.z * w;
+          v.w += y.w * w;
+        }
+        write(r, d, v, best, sum);
+      }
+      cluster_sync();  // no block leaves while another reads its sums
+    }
+    if (following.g < g1) store_q();
+    __syncthreads();  // the sums are free, and q is there for the next segment
+    seg = following;
   } while (seg.g < g1);
   if (dead)  // let this warp's copies land before it exits
     for (; pending > 0; --pending) {
@@ -706,9 +824,9 @@ __global__ void __launch_bounds__(1024) k_merge(const AttnArgs a, int rows_per_s
   const int hr_count = a.hkv * a.row_groups, b = blockIdx.x / hr_count, hr = blockIdx.x % hr_count;
   const int r = blockIdx.y * rows_here + row_here, rr = hr % a.row_groups * rows_per_segment + r;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int chunk = a.plan[0], before = a.plan[1 + b], tiles = a.plan[2 + b] - before;
-  const int begin = before * hr_count + hr * tiles, end = begin + tiles;
-  const int c0 = tiles ? begin / chunk : 0, c1 = tiles ? (end - 1) / chunk : -1;
+  const int chunk = a.plan[0], before = a.plan[1 + b], places = a.plan[2 + b] - before, tiles = places ? places - a.pad : 0;
+  const int begin = before * hr_count + hr * places;
+  const int c0 = tiles ? begin / chunk : 0, c1 = tiles ? (begin + tiles - 1) / chunk : -1;
   if (c0 == c1) return;  // one block held it all
   const bool real = r < rows_per_segment && rr < a.T * a.group;
   float best = -INFINITY, sum = 0.0f;
@@ -762,8 +880,20 @@ __global__ void __launch_bounds__(1024) k_merge(const AttnArgs a, int rows_per_s
 
 using sn::kv::need_ok;
 
+// How many blocks share a segment that is not cut from the line, 0 to cut the line.  Where the
+// tables hold few tiles, the blocks of one cluster take a segment and join through distributed
+// shared memory: one launch, no workspace.  A cluster grows while its blocks hold more than
+// about a tile a warp and the grid stays in one wave (8 sequences x 1024 keys, one KV head:
+// 12.3 us in one block each, 14.5 us from the line, 8.4 us in clusters of 8); more than four
+// such rounds a block go to the line, which balances them.
+int direct_blocks(int64_t segments, int64_t tiles, int resident) {
+  int blocks = 1;
+  while (blocks < 8 && tiles > blocks * 6 && segments * blocks * 2 <= resident) blocks *= 2;
+  return tiles <= blocks * 24 ? blocks : 0;
+}
+
 template <class T, int D, int NT>
-void launch(const AttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, cudaStream_t st) {
+void launch(AttnArgs a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st) {
   using L = Layout<D, NT>;
   auto kernel = k_attention<T, D, NT>;
   static std::atomic<uint64_t> ready{0};  // devices that allow the kernel its shared memory
@@ -775,14 +905,34 @@ void launch(const AttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int
             "paged_decode_attention");
     ready.fetch_or(bit);
   }
-  if (a.direct) blocks = a.n * a.hkv * a.row_groups;
+  const int segments = a.n * a.hkv * a.row_groups;
+  int blocks = segments * std::max(a.direct, 1);
+  if (!a.direct) {
+    a.pad = kPadRounds * L::kWarps;
+    const int places = segments * ((a.width * a.page_size + kTile - 1) / kTile + a.pad);  // at most
+    blocks = std::min(a.resident, (places + L::kWarps - 1) / L::kWarps);
+  }
+  if (a.direct > 1) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(blocks);
+    config.blockDim = dim3(L::kThreads);
+    config.dynamicSmemBytes = L::kBytes;
+    config.stream = st;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim = {unsigned(a.direct), 1, 1};
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    need_ok(cudaLaunchKernelEx(&config, kernel, mk, mv, a), "paged_decode_attention launch");
+    return;
+  }
   kernel<<<blocks, L::kThreads, L::kBytes, st>>>(mk, mv, a);
   need_ok(cudaGetLastError(), "paged_decode_attention launch");
   if (a.direct) return;
 
   // pieces a segment is likely cut into, four of them a group
-  const int segments = a.n * a.hkv * a.row_groups, rows = std::min(L::kRows, a.T * a.group);
-  const int pieces = std::min(blocks / segments + 2, a.width * a.page_size / kTile / L::kWarps + 2);
+  const int rows = std::min(L::kRows, a.T * a.group);
+  const int pieces = std::min(a.resident / segments + 2, a.width * a.page_size / kTile / L::kWarps + 2);
   int groups = 1;
   while (groups < 32 && groups * 4 < pieces) groups *= 2;
   int rows_here = 1;
@@ -802,11 +952,10 @@ void launch(const AttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int
 }
 
 template <class T, int D>
-void launch_rows(const AttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int nt, int blocks,
-                 cudaStream_t st) {
-  if (nt == 1) launch<T, D, 1>(a, mk, mv, blocks, st);
-  else if (nt == 2) launch<T, D, 2>(a, mk, mv, blocks, st);
-  else launch<T, D, 4>(a, mk, mv, blocks, st);
+void launch_rows(const AttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int nt, cudaStream_t st) {
+  if (nt == 1) launch<T, D, 1>(a, mk, mv, st);
+  else if (nt == 2) launch<T, D, 2>(a, mk, mv, st);
+  else launch<T, D, 4>(a, mk, mv, st);
 }
 
 }  // namespace
@@ -869,7 +1018,7 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> KvPool::attention(const at::Te
   const int64_t rows = T * (hq / heads);
   const int nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
   const int64_t row_groups = (rows + 8 * nt - 1) / (8 * nt), segments = n * heads * row_groups;
-  need(segments * ((tables.size(1) * page_size + kTile - 1) / kTile) < (int64_t(1) << 30),
+  need(segments * ((tables.size(1) * page_size + kTile - 1) / kTile + 8) < (int64_t(1) << 30),
        "the sequences' tables, KV heads and query rows together are too large for one call");
   if (out)
     need(out->sizes() == q.sizes() && out->scalar_type() == q.scalar_type() && out->is_contiguous() &&
@@ -893,8 +1042,8 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> KvPool::attention(const at::Te
     mapped_ = true;
   }
   // two blocks of four warps fill an SM's shared memory
-  const int blocks = 2 * at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  const int64_t parts = 2 * int64_t(blocks) * 8 * nt;
+  const int resident = 2 * at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  const int64_t parts = 2 * int64_t(resident) * 8 * nt;  // two pieces a block
   at::Tensor work = at::empty({parts * dim + parts * 2 + n + 2}, k_scale.options());
   AttnArgs a{};
   a.part = work.data_ptr<float>();
@@ -914,6 +1063,7 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> KvPool::attention(const at::Te
   a.table_row = tables.stride(0);
   a.pages = int(pages);
   a.n = int(n);
+  a.resident = resident;
   a.T = int(T);
   a.hq = int(hq);
   a.hkv = heads;
@@ -921,16 +1071,16 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> KvPool::attention(const at::Te
   a.row_groups = int(row_groups);
   a.page_size = page_size;
   a.page_shift = __builtin_ctz(page_size);
-  a.direct = tables.size(1) * page_size <= kDirectTiles * kTile;
   a.width = int(tables.size(1));
   a.window = int(window);
   a.scale_log2 = float(scale * 1.4426950408889634);
+  a.direct = direct_blocks(segments, (tables.size(1) * page_size + kTile - 1) / kTile, resident);
   if (q.scalar_type() == at::kBFloat16) {
-    if (dim == 128) launch_rows<__nv_bfloat16, 128>(a, k_map_, v_map_, nt, blocks, stream());
-    else launch_rows<__nv_bfloat16, 64>(a, k_map_, v_map_, nt, blocks, stream());
+    if (dim == 128) launch_rows<__nv_bfloat16, 128>(a, k_map_, v_map_, nt, stream());
+    else launch_rows<__nv_bfloat16, 64>(a, k_map_, v_map_, nt, stream());
   } else {
-    if (dim == 128) launch_rows<__half, 128>(a, k_map_, v_map_, nt, blocks, stream());
-    else launch_rows<__half, 64>(a, k_map_, v_map_, nt, blocks, stream());
+    if (dim == 128) launch_rows<__half, 128>(a, k_map_, v_map_, nt, stream());
+    else launch_rows<__half, 64>(a, k_map_, v_map_, nt, stream());
   }
   return {o, lse};
 }
