@@ -62,6 +62,8 @@ def parse_args(argv=None):
     p.add_argument("--batch", type=int, default=8, help="decode: sequences per step")
     p.add_argument("--attention", choices=("auto", "simt", "tcgen05"), default="auto",
                    help="decode: attention kernel (auto: tensor cores where their cluster merge fits one wave or from 32 sequence-head pairs)")
+    p.add_argument("--kv-cache", choices=("bf16", "fp8"), default="bf16",
+                   help="decode: contiguous bf16 cache, or paged e4m3 pages with a scale for each page and KV head")
     p.add_argument("--layers", type=int, default=80, help="decode: decoder layers")
     p.add_argument("--fused-norm-tokens", type=int, nargs="*", default=[1, 8, 32, 128, 256],
                    help="ours: also time the fused all-reduce + residual + RMSNorm at these token counts "

@@ -44,6 +44,8 @@ class KvPool {
                                                               const at::Tensor& lengths, double scale, int64_t window,
                                                               const c10::optional<at::Tensor>& out, bool want_lse);
 
+  int attention_launches(int64_t sequences, int64_t tokens, int64_t hq, int64_t width) const;
+
   at::Tensor k, v, k_scale, v_scale;
   at::Tensor err;  // one int32: nonzero after a wait of the attention kernel ran out
   int64_t pages;

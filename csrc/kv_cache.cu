@@ -527,6 +527,8 @@ void register_kv_cache(py::module_& m) {
            py::arg("v_out") = py::none())
       .def("attention", &KvPool::attention, py::arg("q"), py::arg("block_tables"), py::arg("lengths"),
            py::arg("scale"), py::arg("window"), py::arg("out") = py::none(), py::arg("want_lse") = false)
+      .def("attention_launches", &KvPool::attention_launches, py::arg("sequences"), py::arg("tokens"),
+           py::arg("heads"), py::arg("width"))
       .def_readonly("k", &KvPool::k)
       .def_readonly("v", &KvPool::v)
       .def_readonly("k_scale", &KvPool::k_scale)

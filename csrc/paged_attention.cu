@@ -991,6 +991,15 @@ CUtensorMap KvPool::make_map(const at::Tensor& codes) const {
   return map;
 }
 
+int KvPool::attention_launches(int64_t sequences, int64_t tokens, int64_t hq, int64_t width) const {
+  need_cuda();
+  const int64_t rows = tokens * (hq / heads);
+  const int nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  const int64_t segments = sequences * heads * ((rows + 8 * nt - 1) / (8 * nt));
+  const int resident = 2 * at::cuda::getDeviceProperties(k.device().index())->multiProcessorCount;
+  return direct_blocks(segments, (width * page_size + kTile - 1) / kTile, resident) ? 1 : 2;
+}
+
 std::tuple<at::Tensor, c10::optional<at::Tensor>> KvPool::attention(const at::Tensor& q, const at::Tensor& tables,
                                                                     const at::Tensor& lengths, double scale,
                                                                     int64_t window,

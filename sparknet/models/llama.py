@@ -19,6 +19,11 @@ SwiGLU runs in the gate/up GEMM's epilogue; ``gemm="cublas"`` (the default of th
 NCCL control arm) uses ``torch.mm`` and a separate SwiGLU kernel.  Attention, RoPE +
 KV-cache writes, the norms and the argmax are this package's kernels.  A decode step
 is one CUDA graph replay.
+
+``kv_cache="fp8"`` keeps keys and values in paged 8-bit caches (one page table for all
+layers, ``page_size`` tokens a page) instead of one bf16 block a sequence: each step
+plans its pages on the GPU, appends with RoPE and quantisation in one kernel a layer,
+and attends over the pages.
 """
 
 from __future__ import annotations
@@ -32,6 +37,9 @@ import torch.distributed as dist
 from .. import _native
 from ..ops.attention import VARIANTS as ATTENTION_VARIANTS
 from ..ops.decode_gemm import INTERLEAVE_ROWS, DecodeGemm
+from ..ops.kv_cache import Fp8KVCache, kv_append, rope_kv_append
+from ..ops.paged_attention import paged_decode_attention
+from ..ops.paging import PageTable
 
 
 @dataclass(frozen=True)
@@ -71,7 +79,7 @@ class TPLlama:
 
     def __init__(self, cfg: LlamaConfig, *, rank: int, world: int, device, batch: int, max_len: int,
                  comm: str = "sparknet", runtime=None, group=None, seed: int = 0, gemm: str | None = None,
-                 pdl: bool = True, attention: str = "auto"):
+                 pdl: bool = True, attention: str = "auto", kv_cache: str = "bf16", page_size: int = 64):
         if cfg.heads % world or cfg.kv_heads % world or cfg.ffn % world or cfg.vocab % world:
             raise ValueError(f"model does not shard evenly over {world} GPUs")
         if comm not in ("sparknet", "nccl"):
@@ -85,6 +93,11 @@ class TPLlama:
             raise ValueError("the FFN shard must be a multiple of 64 features")
         if attention not in ATTENTION_VARIANTS:
             raise ValueError(f"attention must be one of {sorted(ATTENTION_VARIANTS)}")
+        if kv_cache not in ("bf16", "fp8"):
+            raise ValueError("kv_cache must be 'bf16' or 'fp8'")
+        if kv_cache == "fp8" and attention != "auto":
+            raise ValueError("the fp8 cache has one attention kernel: attention must be 'auto'")
+        self.kv_cache = kv_cache
         self.gemm = gemm
         self.attention = attention
         self.cfg, self.rank, self.world, self.device = cfg, rank, world, torch.device(device)
@@ -108,9 +121,18 @@ class TPLlama:
                 "ln2": torch.ones(H, dtype=torch.bfloat16, device=dev),
                 "wgu": _normal((2 * self.f, H), dev, generator=gen),   # [64 gate; 64 up] row blocks
                 "wdown": _normal((H, self.f), dev, generator=gen),
-                "k": torch.zeros((batch, max_len, self.hkv, D), dtype=torch.bfloat16, device=dev),
-                "v": torch.zeros((batch, max_len, self.hkv, D), dtype=torch.bfloat16, device=dev),
             })
+        pages = -(-max_len // page_size)
+        self.table = None
+        if kv_cache == "fp8":
+            self.table = PageTable(batch * pages, page_size=page_size, max_requests=batch, max_pages=pages, device=dev)
+            self.one_each = torch.ones(batch, dtype=torch.int32, device=dev)
+        for layer in self.layers:
+            if kv_cache == "fp8":
+                layer["cache"] = Fp8KVCache(batch * pages, self.hkv, page_size=page_size, head_dim=D, device=dev)
+            else:
+                layer["k"], layer["v"] = (torch.zeros((batch, max_len, self.hkv, D), dtype=torch.bfloat16, device=dev)
+                                          for _ in range(2))
         self.norm = torch.ones(H, dtype=torch.bfloat16, device=dev)
         self.lm_head = _normal((self.v, H), dev, generator=gen)
         inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, D // 2, dtype=torch.float64) * 2 / D))
@@ -143,7 +165,15 @@ class TPLlama:
         """Random KV entries for ``prompt_len`` positions (a prefill stand-in) and the
         decode position right after them."""
         gen = torch.Generator(device=self.device).manual_seed(seed * 7 + self.rank)
+        if self.table is not None:  # every sequence starts anew
+            rows = self.batch * prompt_len
+            plan = self.table.extend(torch.full_like(self.lengths, prompt_len), rows,
+                                     torch.ones(self.batch, dtype=torch.bool, device=self.device))
         for layer in self.layers:
+            if self.table is not None:
+                k, v = (_normal((rows, self.hkv, self.cfg.head_dim), self.device, 1.0, gen) for _ in range(2))
+                kv_append(layer["cache"], k, v, plan.slots)
+                continue
             layer["k"][:, :prompt_len].normal_(0, 1, generator=gen)
             layer["v"][:, :prompt_len].normal_(0, 1, generator=gen)
         self.positions.fill_(prompt_len)
@@ -189,16 +219,24 @@ class TPLlama:
         torch.index_select(self.embed, 0, self.tokens, out=self.res)
         C.add_rmsnorm(self.res, None, None, self.layers[0]["ln1"], self.x, cfg.eps)
         scale = 1.0 / math.sqrt(cfg.head_dim)
+        if self.table is not None:
+            plan = self.table.extend(self.one_each, self.batch)
         for i, L in enumerate(self.layers):
-            if self.gemm == "sparknet":  # RoPE and the KV-cache write in the GEMM epilogue
+            if self.table is not None:
+                self._linear(self.x, L["wqkv"], self.qkv)
+                rope_kv_append(L["cache"], self.qkv, self.cos, self.sin, plan.positions, plan.slots, self.q)
+                paged_decode_attention(self.q, L["cache"], self.table.block_tables, self.table.lengths, scale=scale,
+                                       out=self.attn)
+            elif self.gemm == "sparknet":  # RoPE and the KV-cache write in the GEMM epilogue
                 self.mm.qkv_rope(self.x, L["wqkv"], self.cos, self.sin, self.positions, self.q, L["k"], L["v"],
                                  self.hq, self.hkv)
             else:
                 self._linear(self.x, L["wqkv"], self.qkv)
                 C.rope_qkv_cache(self.qkv, self.cos, self.sin, self.positions, self.q, L["k"], L["v"], self.hq,
                                  self.hkv)
-            C.decode_attention(self.q, L["k"], L["v"], self.lengths, self.attn, self.workspace, self.max_len,
-                               scale, self.pdl, ATTENTION_VARIANTS[self.attention])
+            if self.table is None:
+                C.decode_attention(self.q, L["k"], L["v"], self.lengths, self.attn, self.workspace, self.max_len,
+                                   scale, self.pdl, ATTENTION_VARIANTS[self.attention])
             last = i + 1 == len(self.layers)
             nxt = self.norm if last else self.layers[i + 1]["ln1"]
             self._linear(self.attn.view(self.batch, -1), L["wo"], self.partial)
@@ -219,14 +257,16 @@ class TPLlama:
         """Capture one decode step into a CUDA graph (after one eager warm-up step)."""
         stream = torch.cuda.Stream(device=self.device)
         stream.wait_stream(torch.cuda.current_stream(self.device))
-        snap = (self.positions.clone(), self.lengths.clone(), self.tokens.clone())
+        state = [self.positions, self.lengths, self.tokens]
+        if self.table is not None:  # the captured step takes the warm-up's pages again
+            state += [self.table.lengths, self.table.free_count]
+        snap = [t.clone() for t in state]
         with torch.cuda.stream(stream):
             self.step_kernels()
         torch.cuda.current_stream(self.device).wait_stream(stream)
         torch.cuda.synchronize(self.device)
-        self.positions.copy_(snap[0])
-        self.lengths.copy_(snap[1])
-        self.tokens.copy_(snap[2])
+        for t, was in zip(state, snap):
+            t.copy_(was)
         g = torch.cuda.CUDAGraph()
         ctx = self.runtime.capture(stream=stream) if self.runtime is not None else _null()
         with torch.cuda.graph(g, stream=stream), ctx:
@@ -243,12 +283,18 @@ class TPLlama:
         """This package's kernel launches in one step (torch index/copy ops and cuBLAS
         GEMMs excluded): per layer attention and two norms (fused with the all-reduce on
         the NVLink arm), plus four GEMMs with RoPE and SwiGLU fused (``gemm="sparknet"``)
-        or the RoPE and SwiGLU kernels (cuBLAS arm)."""
+        or the RoPE and SwiGLU kernels (cuBLAS arm).  The fp8 cache adds the plan, and in each
+        layer the append (in place of RoPE) and the attention's second kernel where it has one."""
         # sparknet: QKV+RoPE, O, gate/up+SwiGLU, down GEMMs; cuBLAS arm: RoPE and SwiGLU kernels
         per_layer = 1 + 2 + (4 if self.gemm == "sparknet" else 2)
+        plan = 0
+        if self.table is not None:
+            plan = 1
+            attend = self.layers[0]["cache"].attention_launches(self.batch, self.hq, self.table.block_tables.shape[1])
+            per_layer += attend - 1 + (1 if self.gemm == "sparknet" else 0)
         own_gather = 1 if (self.world > 1 and self.comm == "sparknet") else 0
         lm_head = 1 if self.gemm == "sparknet" else 0
-        return 1 + self.cfg.layers * per_layer + lm_head + 1 + own_gather
+        return 1 + plan + self.cfg.layers * per_layer + lm_head + 1 + own_gather
 
 
 class _null:

@@ -65,6 +65,10 @@ class Fp8KVCache:
         """Bytes of the codes and scales."""
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale))
 
+    def attention_launches(self, sequences: int, heads: int, width: int, tokens: int = 1) -> int:
+        """Kernels that ``paged_decode_attention`` launches for these shapes: 1 or 2."""
+        return self._pool.attention_launches(sequences, tokens, heads, width)
+
     def check(self) -> None:
         """Synchronise and raise if an attention kernel over this cache gave up on a load."""
         if self.device.type == "cuda":

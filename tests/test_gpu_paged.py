@@ -647,3 +647,47 @@ def test_attention_offsets_past_32_bits(device):
     q = torch.randn(1, 1, 16, 128, generator=gen, device=device).to(torch.bfloat16)
     a = check_attention(q, small, torch.arange(3, dtype=torch.int32, device=device)[None], ints([300], device))
     assert torch.equal(a, ops.paged_decode_attention(q, c, tables, ints([300], device)))
+
+
+# -- the model that decodes over it ------------------------------------------------------
+@pytest.mark.parametrize("gemm", ["sparknet", "cublas"])
+def test_tiny_model_over_the_fp8_cache(device, gemm):
+    """A decode step's last attention against the definition over what the last layer's cache
+    holds; graph replay decodes the eager tokens; pages run over a border (page 16)."""
+    from sparknet.models.llama import LlamaConfig, TPLlama
+
+    def model():
+        m = TPLlama(LlamaConfig.tiny(layers=2), rank=0, world=1, device=device, batch=3, max_len=48, gemm=gemm,
+                    kv_cache="fp8", page_size=16)
+        m.fill_prompt_cache(14)
+        m.tokens.copy_(torch.tensor([1, 2, 3], device=device))
+        return m
+
+    m, eager = model(), []
+    for _ in range(5):
+        m.step_kernels()
+        eager.append(m.tokens.tolist())
+    assert m.table.lengths.tolist() == [19] * 3 and int(m.table.free_count) == 9 - 3 * 2
+    want, _, bound = attention_by_definition(m.q[:, None], m.layers[-1]["cache"], m.table.block_tables,
+                                             m.table.lengths)
+    assert bool(((m.attn.double().cpu()[:, None] - want).abs() <= bound).all())
+    g, replayed = model(), []
+    g.capture()
+    for _ in range(5):
+        g.replay()
+        replayed.append(g.tokens.tolist())
+    assert replayed == eager
+    assert g.launches_per_step() > 0
+    g.layers[0]["cache"].check()
+    for _ in range(40):  # past max_len: tokens without slots, nothing grows
+        g.replay()
+    assert g.table.lengths.tolist() == [48] * 3
+    g.release()
+
+
+def test_tiny_model_refuses(device):
+    from sparknet.models.llama import LlamaConfig, TPLlama
+
+    for bad in ({"kv_cache": "int8"}, {"kv_cache": "fp8", "attention": "simt"}, {"kv_cache": "fp8", "page_size": 24}):
+        with pytest.raises(ValueError):
+            TPLlama(LlamaConfig.tiny(layers=1), rank=0, world=1, device=device, batch=1, max_len=48, **bad)
